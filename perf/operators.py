@@ -13,7 +13,6 @@ K/V cache and attends from them:
 """
 from __future__ import annotations
 
-import functools
 import math
 import os
 import sys
@@ -27,7 +26,6 @@ THETA, EPS = 1e6, 1e-6
 SCORES_MAX = 2.2e9  # entries of the padded score matrix of a plain attention: its temporaries fit the card
 
 
-@functools.lru_cache
 def _paged():
     pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "reki-megakernel_amd")
     if pkg not in sys.path:
@@ -238,7 +236,6 @@ def _prepare_rope(c, seed, dev, g):
         slots = torch.randperm(n_pages * c["P"], generator=g, device=dev)[:T]
         s["slots"] = torch.where(torch.arange(T, device=dev) % 16 == 15, -1, slots)
         s["n_pages"] = n_pages
-        s["used"] = s["kp"][:n_pages], s["vp"][:n_pages]  # the pages of a user's cache
     if own:
         s["rope"] = _paged().AxesRotary(HD, _axis_of(c), theta=THETA, q_norm=s["wq"], k_norm=s["wk"], eps=EPS, device=dev)
     return s
@@ -377,7 +374,8 @@ def run(s):
             if "slots" not in s:
                 q, k = s["rope"](s["q"], s["k"], s["pos"])
                 return {"q": q, "k": k}
-            kp, vp = s["used"]
+            N = s["n_pages"]
+            kp, vp = s["kp"][:N], s["vp"][:N]
             return {"q": s["rope"].store(s["q"], s["k"], s["v"], s["pos"], kp, vp, s["slots"]), "k_pages": kp, "v_pages": vp}
         return _paged().page_attend(s["q"], s["kp"], s["vp"], s["table"], s["cu"], s["kv_len"], max_q=s["max_q"], scale=s["scale"],
                                     causal=s["causal"], window=s["window"], sinks=s["sinks"], out=s["out"])
