@@ -437,6 +437,11 @@ typedef struct {
 int64_t mkx_page_attend_workspace(const mkx_attend_args* args);
 int mkx_page_attend(const mkx_attend_args* args, void* stream);
 
+/* The same for a step of mkx_page_map that may have refused requests: granted [B] (its output; NULL: all are) marks with 0 the
+ * slots whose tokens are not in the cache. Their queries see nothing and their rows are zeros; mkx_page_attend would give them
+ * attention at positions kv_len[b] - n + i among tokens that are not theirs. */
+int mkx_page_attend_granted(const mkx_attend_args* args, const int32_t* granted, void* stream);
+
 /* Synchronisation micro-benchmarks (no handle). Reference: the barrier-only kernel _barrier_only
  * (src/tune_mk.py:28-33), timed at :66-68 to price the reference's grid barrier (results/opt/tune/v5.json:3-4).
  * MKX_PROBE_BARRIER: every workgroup of a one-per-CU grid passes n grid barriers (this library's barrier,

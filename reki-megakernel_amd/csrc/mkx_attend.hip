@@ -78,19 +78,7 @@ unsigned long long next_stamp() {
   return (seed + 2 * g_stamp.fetch_add(1, std::memory_order_relaxed)) * 0x9E3779B97F4A7C15ull;  // odd times odd: never 0
 }
 
-}  // namespace
-
-extern "C" {
-
-int64_t mkx_page_attend_workspace(const mkx_attend_args* a) {
-  const char* me = "mkx_page_attend_workspace";
-  int shift, cus;
-  if (check_sizes(a, me, &shift) != MKX_OK || cus_here(me, &cus) != MKX_OK) return -1;
-  return ws_of(a, launch_of(a, shift, cus));
-}
-
-int mkx_page_attend(const mkx_attend_args* a, void* stream) {
-  const char* me = "mkx_page_attend";
+int attend(const char* me, const mkx_attend_args* a, const int32_t* granted, void* stream) {
   int shift;
   const int rc = check_sizes(a, me, &shift);
   if (rc != MKX_OK) return rc;
@@ -110,6 +98,7 @@ int mkx_page_attend(const mkx_attend_args* a, void* stream) {
   const int no_cus = cus_here(me, &cus);
   if (no_cus != MKX_OK) return no_cus;
   AttendLaunch L = launch_of(a, shift, cus);
+  L.granted = granted;
   if (a->ws_bytes < ws_of(a, L)) return set_error(MKX_EINVAL, me, "ws_bytes smaller than mkx_page_attend_workspace()");
   try {
     L.stamp = next_stamp();
@@ -121,6 +110,23 @@ int mkx_page_attend(const mkx_attend_args* a, void* stream) {
                                             : (a->HD == 128 ? go<FP16, 128>(*a, L, st) : go<FP16, 64>(*a, L, st));
   if (e != hipSuccess) return set_error(MKX_EHIP, me, hipGetErrorString(e));
   return MKX_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t mkx_page_attend_workspace(const mkx_attend_args* a) {
+  const char* me = "mkx_page_attend_workspace";
+  int shift, cus;
+  if (check_sizes(a, me, &shift) != MKX_OK || cus_here(me, &cus) != MKX_OK) return -1;
+  return ws_of(a, launch_of(a, shift, cus));
+}
+
+int mkx_page_attend(const mkx_attend_args* a, void* stream) { return attend("mkx_page_attend", a, nullptr, stream); }
+
+int mkx_page_attend_granted(const mkx_attend_args* a, const int32_t* granted, void* stream) {
+  return attend("mkx_page_attend_granted", a, granted, stream);
 }
 
 }  // extern "C"

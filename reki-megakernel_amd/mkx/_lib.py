@@ -19,7 +19,8 @@ EXPORTS = ("mkx_create", "mkx_run", "mkx_check", "mkx_barriers", "mkx_set_profil
            "mkx_last_error", "mkx_status_string", "mkx_abi_version", "mkx_ring_append", "mkx_source_create", "mkx_source_run", "mkx_source_destroy",
            "mkx_modulations", "mkx_set_spin_limit", "mkx_source_run_noalloc", "mkx_modulation_input", "mkx_modulation_input_ws",
            "mkx_probe",
-           "mkx_set_operand_shift", "mkx_page_map", "mkx_rope_axes", "mkx_page_attend", "mkx_page_attend_workspace")
+           "mkx_set_operand_shift", "mkx_page_map", "mkx_rope_axes", "mkx_page_attend", "mkx_page_attend_workspace",
+           "mkx_page_attend_granted")
 PROBE_BARRIER, PROBE_HANDOFF = 0, 1
 BF16, FP16 = 0, 1
 MAX_SLOTS = 2048
@@ -171,6 +172,7 @@ def lib() -> ctypes.CDLL:
         L.mkx_page_map.argtypes = [ctypes.POINTER(MkxPageMapArgs), _vp]
         L.mkx_rope_axes.argtypes = [ctypes.POINTER(MkxRopeArgs), _vp]
         L.mkx_page_attend.argtypes = [ctypes.POINTER(MkxAttendArgs), _vp]
+        L.mkx_page_attend_granted.argtypes = [ctypes.POINTER(MkxAttendArgs), _vp, _vp]
         L.mkx_page_attend_workspace.argtypes = [ctypes.POINTER(MkxAttendArgs)]
         L.mkx_page_attend_workspace.restype = ctypes.c_int64
         _LIB = L

@@ -309,12 +309,13 @@ class AxesRotary:
 
 def page_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, cu: torch.Tensor,
                 kv_len: torch.Tensor, *, max_q: int | None = None, scale: float | None = None, causal: bool = True, window: int = 0,
-                sinks: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+                sinks: int = 0, out: torch.Tensor | None = None, granted: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of new tokens over the paged cache: q [T, NQ, head_dim], slot b's tokens at cu[b] .. cu[b + 1] - 1 and at the
     end of its kv_len[b] cached tokens (their own k and v stored before). causal with ``window`` > 0: a token sees the last
     ``window`` tokens up to itself and the request's first ``sinks``. ``max_q``: a bound of the chunks' lengths that the
     caller knows (1 for answered tokens), which shapes the launch only. ``out``: where the result goes; rows behind the
-    last slot's tokens are left as they are there (and unset without it)."""
+    last slot's tokens are left as they are there (and unset without it). ``granted`` (``PageMap.granted``): slots with 0 were
+    refused their tokens, which are not in the cache; their rows are zeros."""
     shape = q.shape
     hd = shape[2] if len(shape) == 3 else 0
     if hd not in (64, 128):
@@ -322,9 +323,9 @@ def page_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
     index = q.get_device()
     if index < 0:
         raise ValueError(f"q is on {q.device}: the paged cache sits on a GPU")
-    for t in (k_pages, v_pages, table, cu, kv_len, out):
+    for t in (k_pages, v_pages, table, cu, kv_len, out, granted):
         if t is not None and t.get_device() != index:
-            require_device(q.device, k_pages=k_pages, v_pages=v_pages, table=table, cu=cu, kv_len=kv_len, out=out)
+            require_device(q.device, k_pages=k_pages, v_pages=v_pages, table=table, cu=cu, kv_len=kv_len, out=out, granted=granted)
     dt = q.dtype
     q, shape, qs, qh, qp = _heads(q, "q", hd)
     T, NQ, _ = shape
@@ -337,6 +338,7 @@ def page_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
     B = n[0]
     _ints(kv_len, (B,), "kv_len")
     _ints(cu, (B + 1,), "cu")
+    has = 0 if granted is None else _ints(granted, (B,), "granted").data_ptr()
     n, strides = table.shape, table.stride()
     if len(n) != 2 or n[0] != B or n[1] < 1 or table.dtype != torch.int32 or strides[1] != 1 or strides[0] < n[1]:
         raise ValueError(f"table must be [{B}, pages] int32 with contiguous rows, got {tuple(n)} {table.dtype}")
@@ -355,21 +357,21 @@ def page_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
         a = _attend_args(T, B, NQ, NK, hd, cols, NP, P, _DTYPES[dt], 1 if causal else 0, window, sinks, min(max_q, T), scale, qp, op, qs, qh, os, oh,
                          kp, vp, ps, pr, ph, table.data_ptr(), rows, cu.data_ptr(), kv_len.data_ptr(), 0, 0)
         if _device() == index:
-            _attend(a, index)
+            _attend(a, has, index)
         else:
             with torch.cuda.device(index):
-                _attend(a, index)
+                _attend(a, has, index)
     return out
 
 
-def _attend(a: MkxAttendArgs, index: int) -> None:
+def _attend(a: MkxAttendArgs, granted: int, index: int) -> None:
     L, ref = lib(), ctypes.byref(a)
     n = L.mkx_page_attend_workspace(ref)
     if n < 0:
         check(EINVAL, "mkx_page_attend_workspace")
     ws = torch.empty(n, dtype=torch.uint8, device=index)  # of this call and its stream alone
     a.ws, a.ws_bytes = ws.data_ptr(), n
-    rc = L.mkx_page_attend(ref, _stream(index))
+    rc = L.mkx_page_attend_granted(ref, granted, _stream(index)) if granted else L.mkx_page_attend(ref, _stream(index))
     if rc != OK:
         check(rc, "mkx_page_attend")
 
@@ -395,4 +397,5 @@ class PagedCache:
         return rope.store(q, k, v, pos, self.k[layer], self.v[layer], m.slots, q_out=q_out)
 
     def attend(self, layer: int, q: torch.Tensor, m: PageMap, **how) -> torch.Tensor:
-        return page_attend(q, self.k[layer], self.v[layer], m.table, m.cu, m.kv_len, **how)
+        """``page_attend`` of the step; rows of requests that it did not grant are zeros."""
+        return page_attend(q, self.k[layer], self.v[layer], m.table, m.cu, m.kv_len, granted=m.granted, **how)

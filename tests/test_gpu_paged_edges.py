@@ -1,0 +1,105 @@
+"""The paged cache's operators in calls beside the ordinary ones: requests that were not granted, positions and weights of other
+types, sizes at the launch's limits, the attention's other kernel."""
+import random
+
+import pytest
+import torch
+
+from mkx.paged import AxesRotary, PagedCache
+
+from _paged_ref import attend_ref
+from test_gpu_paged import BF, DEV, FP, Att, _near, i32
+
+pytestmark = pytest.mark.gpu
+torch.set_grad_enabled(False)
+
+
+# ---- requests that were not granted -----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("how", [dict(), dict(max_q=40), dict(causal=False), dict(window=20, sinks=3)])
+@pytest.mark.parametrize("graph", [False, True])
+def test_rows_of_refused_requests_are_zero(how, graph):
+    """Steps whose pool or whose table row runs out: the refused requests' rows are zeros, the others' their attention, and
+    rows behind the tokens stay; a request refused once is served when its pages are there."""
+    NQ, NK, HD, B, P, cap = 4, 2, 64, 5, 16, 120
+    cache = PagedCache(1, NK, HD, 9, slots=B, table_cols=4, max_tokens=cap, page_rows=P, device=DEV)
+    for t in cache.k + cache.v:
+        t.fill_(float("nan"))
+    rope = AxesRotary(HD, [0] * (HD // 2), device=DEV)
+    add, done = i32([0] * B), i32([0] * B)
+    g = torch.Generator().manual_seed(3)
+    x, pos = torch.zeros(cap, NQ + 2 * NK, HD, dtype=BF, device=DEV), torch.arange(cap, dtype=torch.int32, device=DEV)
+    out = torch.zeros(cap, NQ, HD, dtype=BF, device=DEV)
+    q = torch.zeros(cap, NQ, HD, dtype=BF, device=DEV)
+
+    def step():
+        m = cache.append(add, done)
+        a, k, v = x.split([NQ, NK, NK], 1)
+        cache.store(0, rope, a, k, v, pos, m, q_out=q)
+        cache.attend(0, q, m, out=out, **how)
+        return m
+
+    graphs, maps = [], []
+    if graph:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(), step()
+        torch.cuda.current_stream().wait_stream(side)
+        for _ in range(2):
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr):
+                maps.append(step())
+            graphs.append(gr)
+    # 9 pages of 16: 30 + 20 + 1 + 0 + 40 tokens take 2 + 2 + 1 + 0 + 3; slot 0 then wants 2 more, one too many, slot 2 more than its
+    # table row; slot 1 ends, and slot 0 has its pages
+    steps = [([30, 20, 1, 0, 40], [0] * 5, [1, 1, 1, 1, 1]), ([33, 5, 1, 0, 2], [0] * 5, [0, 1, 1, 1, 1]),
+             ([0, 0, 64, 0, 1], [0, 1, 0, 0, 0], [1, 0, 0, 1, 1]), ([33, 3, 1, 0, 1], [0] * 5, [1, 1, 1, 1, 1])]
+    for i, (a, d, granted) in enumerate(steps):
+        add.copy_(i32(a)), done.copy_(i32(d))
+        x.copy_(torch.randn(x.shape, generator=g).to(BF))
+        out.fill_(9.0)
+        if graph:
+            graphs[i % 2].replay()
+            m = maps[i % 2]
+        else:
+            m = step()
+        torch.cuda.synchronize()
+        assert m.granted.tolist() == granted, i
+        cu, n, table = m.cu.tolist(), m.kv_len.tolist(), m.table.tolist()
+        got, qc = out.cpu(), q.cpu()
+        assert bool((got[cu[-1]:] == 9).all())
+        for b in range(B):
+            lo, hi = cu[b], cu[b + 1]
+            if not granted[b]:
+                assert bool((got[lo:hi] == 0).all()), (i, b)
+                continue
+            held = table[b][: -(-n[b] // P)]
+            k, v = (t[0][held].flatten(0, 1)[: n[b]].cpu() for t in (cache.k, cache.v))
+            o, tol = attend_ref(qc[lo:hi], k, v, how.get("causal", True), how.get("window", 0), how.get("sinks", 0), HD ** -0.5)
+            _near(got[lo:hi], o, tol, (i, b))
+
+
+@pytest.mark.parametrize("max_q,B", [(1, 3), (None, 3), (None, 70), (None, 2048)])
+def test_attention_of_some_granted_requests(max_q, B):
+    """Every plan: requests in a wave's registers, tiles in them, a workgroup's plan, a workgroup for each tile."""
+    rng = random.Random(B)
+    nq = [rng.choice([1, 2, 0, 70 if B == 3 else 3]) for _ in range(B)]
+    nq[0] = 1
+    n = [x + rng.choice([0, 5, 40]) for x in nq]
+    t = Att(nq, n, 8, 1, 64, 16, FP, seed=B, lead=2, tail=3)
+    granted = [rng.choice([0, 1, -5]) for _ in range(B)]
+    granted[-1] = 0
+    out = torch.full_like(t.qd, 7.0)
+    t.run(out=out, max_q=max_q, granted=i32(granted))
+    full = t.run(max_q=max_q)
+    for b in range(B):
+        lo, hi = t.cu_l[b], t.cu_l[b + 1]
+        assert torch.equal(out[lo:hi], full[lo:hi] if granted[b] else torch.zeros_like(full[lo:hi])), b
+    assert bool((out[:2] == 7).all()) and bool((out[-3:] == 7).all())
+    with pytest.raises(ValueError, match="granted"):
+        t.run(granted=i32(granted + [1]))
+    with pytest.raises(ValueError, match="granted"):
+        t.run(granted=i32(granted).long())
+    with pytest.raises(ValueError, match="granted is on cpu"):
+        t.run(granted=torch.ones(B, dtype=torch.int32))
