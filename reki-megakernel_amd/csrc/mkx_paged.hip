@@ -21,6 +21,29 @@ int page_shift(int rows) {  // -1: not a page size
   return -1;
 }
 
+// The n tokens (or as many as there are) from t0 on
+mkx_rope_args rope_from(mkx_rope_args a, int64_t t0, int64_t n) {
+  auto skip = [&](const void* p, int64_t stride) { return (void*)((uintptr_t)p + 2 * (uintptr_t)(t0 * stride)); };
+  a.T = (int)(a.T - t0 < n ? a.T - t0 : n);
+  a.q = skip(a.q, a.q_stride_t), a.k = skip(a.k, a.k_stride_t), a.v = skip(a.v, a.v_stride_t);
+  a.q_out = skip(a.q_out, a.qo_stride_t), a.k_out = skip(a.k_out, a.ko_stride_t);
+  a.pos += t0;
+  if (a.slots != nullptr) a.slots += t0;
+  return a;
+}
+
+hipError_t launch_rope(const mkx_rope_args& a, int shift, int tok, hipStream_t st) {
+  const dim3 grid((unsigned)((a.T + tok - 1) / tok)), block(ROPE_BLOCK);
+  if (a.dtype == MKX_BF16) {
+    if (a.HD == 128) hipLaunchKernelGGL((rope_kernel<BF16, 128>), grid, block, 0, st, a, shift, tok);
+    else hipLaunchKernelGGL((rope_kernel<BF16, 64>), grid, block, 0, st, a, shift, tok);
+  } else {
+    if (a.HD == 128) hipLaunchKernelGGL((rope_kernel<FP16, 128>), grid, block, 0, st, a, shift, tok);
+    else hipLaunchKernelGGL((rope_kernel<FP16, 64>), grid, block, 0, st, a, shift, tok);
+  }
+  return hipGetLastError();
+}
+
 }  // namespace
 
 extern "C" {
@@ -99,16 +122,9 @@ int mkx_rope_axes(const mkx_rope_args* a, void* stream) {
   // each 27.6, with half as many 21.6; 1100 tokens of 16 + 2 heads: one token each 4.5 us, four 5.4)
   const int units = (a->NQ + (store ? 2 : 1) * a->NK) * (a->HD / 16), fit = ROPE_BLOCK / units;
   const int tok = fit < 1 ? 1 : fit < ROPE_TOK ? fit : ROPE_TOK;
-  const dim3 grid((unsigned)((a->T + tok - 1) / tok)), block(ROPE_BLOCK);
-  hipStream_t st = (hipStream_t)stream;
-  if (a->dtype == MKX_BF16) {
-    if (a->HD == 128) hipLaunchKernelGGL((rope_kernel<BF16, 128>), grid, block, 0, st, *a, shift, tok);
-    else hipLaunchKernelGGL((rope_kernel<BF16, 64>), grid, block, 0, st, *a, shift, tok);
-  } else {
-    if (a->HD == 128) hipLaunchKernelGGL((rope_kernel<FP16, 128>), grid, block, 0, st, *a, shift, tok);
-    else hipLaunchKernelGGL((rope_kernel<FP16, 64>), grid, block, 0, st, *a, shift, tok);
-  }
-  HIPRC(me, hipGetLastError());
+  // A launch has fewer than 2^32 threads (a larger grid wraps around without an error): 2^23 workgroups at a time
+  const int64_t most = (int64_t)tok << 23;
+  for (int64_t t0 = 0; t0 < a->T; t0 += most) HIPRC(me, launch_rope(rope_from(*a, t0, most), shift, tok, (hipStream_t)stream));
   return MKX_OK;
 }
 

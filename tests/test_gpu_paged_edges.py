@@ -5,7 +5,7 @@ import random
 import pytest
 import torch
 
-from mkx.paged import AxesRotary, PagedCache
+from mkx.paged import AxesRotary, PagedCache, page_attend
 
 from _paged_ref import attend_ref
 from test_gpu_paged import BF, DEV, FP, Att, _near, i32
@@ -103,3 +103,26 @@ def test_attention_of_some_granted_requests(max_q, B):
         t.run(granted=i32(granted).long())
     with pytest.raises(ValueError, match="granted is on cpu"):
         t.run(granted=torch.ones(B, dtype=torch.int32))
+
+
+# ---- launches of the largest sizes ------------------------------------------------------------------------------------------------
+
+def test_rope_of_more_tokens_than_a_launch_has_workgroups():
+    """2^24 workgroups of 256 threads are one more than a launch takes; 33 heads of 64, stored, are a token each."""
+    HD, NK, T, P = 64, 33, (1 << 24) + 70, 16
+    at = [0, 1, (1 << 23) - 1, 1 << 23, (1 << 23) + 1, (1 << 24) - 2, (1 << 24) - 1, 1 << 24, T - 1]
+    rope = AxesRotary(HD, AxesRotary.sections((16, 16)), q_norm=torch.zeros(HD, device=DEV, dtype=BF), device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(4)
+    q, k, v = (torch.randn(1, n, HD, generator=g, device=DEV).to(BF) for n in (1, NK, NK))
+    pos = torch.stack([torch.arange(T, device=DEV), T - torch.arange(T, device=DEV)])
+    slots = torch.full((T,), -1, dtype=torch.int64, device=DEV)
+    slots[at] = torch.arange(len(at), device=DEV) + 3
+    for positions in (pos.int(), pos):
+        kp, vp = (torch.zeros(2, P, NK, HD, dtype=BF, device=DEV) for _ in range(2))
+        out = torch.full((T + 1, 1, HD), 9.0, dtype=BF, device=DEV)
+        rope.store(q.expand(T, 1, HD), k.expand(T, NK, HD), v.expand(T, NK, HD), positions, kp, vp, slots, q_out=out[:T])
+        n = len(at)
+        kw, vw = torch.zeros_like(kp), torch.zeros_like(vp)
+        want = rope.store(q.expand(n, 1, HD), k.expand(n, NK, HD), v.expand(n, NK, HD), positions[:, at].contiguous(), kw, vw, slots[at])
+        assert torch.equal(out[at], want) and torch.equal(kp, kw) and torch.equal(vp, vw)
+        assert bool((out[T] == 9).all()) and bool((out[:T].view(torch.int16) != out[T, 0, 0].view(torch.int16)).any(-1).all())
