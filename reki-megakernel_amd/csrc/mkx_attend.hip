@@ -47,6 +47,9 @@ AttendLaunch launch_of(const mkx_attend_args* a, int shift, int cus) {
   L.G = a->NQ / a->NK;
   const int64_t rows = (int64_t)(a->max_q < a->T ? a->max_q : a->T) * L.G;
   L.bm = rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+  // A launch has fewer than 2^32 threads (a larger grid wraps around without an error): larger tiles for that many rows. With 256
+  // rows there are at most 2^30 / 256 + MKX_MAX_SLOTS * 1024 of them, below 2^23.
+  while (L.bm < 256 && ((int64_t)a->T * L.G / L.bm + a->B) * a->NK >= 1 << 23) L.bm *= 2;
   // Two tiles of 256 rows a CU and more go to workgroups of their own as CUs become free (8192-token prompt of 16 + 2 heads:
   // 285 us against 307 shared out), and so do more tiles than a workgroup can look through.
   const int64_t tiles = (int64_t)a->T * L.G / L.bm + a->B;

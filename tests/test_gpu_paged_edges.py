@@ -126,3 +126,18 @@ def test_rope_of_more_tokens_than_a_launch_has_workgroups():
         want = rope.store(q.expand(n, 1, HD), k.expand(n, NK, HD), v.expand(n, NK, HD), positions[:, at].contiguous(), kw, vw, slots[at])
         assert torch.equal(out[at], want) and torch.equal(kp, kw) and torch.equal(vp, vw)
         assert bool((out[T] == 9).all()) and bool((out[:T].view(torch.int16) != out[T, 0, 0].view(torch.int16)).any(-1).all())
+
+
+@pytest.mark.parametrize("lead", [0, 1 << 28, 1 << 29])
+def test_attention_of_more_rows_than_a_launch_has_workgroups_for(lead):
+    """A q of 2^29 rows, nearly all of them no request's, with max_q = 1: tiles of 64 rows would be 2^23 workgroups of 512."""
+    t = Att([1, 1, 1], [300, 5, 70], 1, 1, 64, 16, BF, seed=2)
+    T = (1 << 29) + 100
+    t.q[:] = t.q[:1].clone()
+    out = torch.empty(T, 1, 64, dtype=BF, device=DEV)  # 64 GiB, nearly none of them touched
+    out[lead: lead + 9] = 4.0
+    page_attend(t.qd[:1].expand(T, 1, 64), t.kp, t.vp, t.table, t.cu + lead, t.kv, max_q=1, out=out)
+    t.check(out[lead: lead + 3])
+    assert bool((out[lead + 3: lead + 9] == 4).all())
+    del out
+    torch.cuda.empty_cache()
