@@ -320,6 +320,8 @@ int mkx_modulation_input_ws(const mkx_modin_args* args, float* ws, void* stream)
  * [n_pages, page_rows, NK, HD]; request slot b owns the pages of row b of the block table, table[b][j] holding its tokens
  * j * page_rows and on. Calls are asynchronous on `stream`, allocate nothing, and can be captured. 16-bit types: */
 typedef enum { MKX_BF16 = 0, MKX_FP16 = 1 } mkx_dtype;
+/* Added to mkx_rope_args.dtype: pos is int64_t (8-byte aligned; beyond 2^53 a position is taken as the nearest double). */
+#define MKX_ROPE_POS64 256
 #define MKX_MAX_SLOTS 2048
 
 /* Block tables and slots of one step, from the requests' lengths. Request slot b has len_in[b] tokens and appends
@@ -361,7 +363,7 @@ int mkx_page_map(const mkx_page_map_args* args, void* stream);
 
 /* Rotary positions of several axes (time, height, width, ...) for q and k, with optional per-head RMS norms, k and v
  * optionally stored in pages. Pair i of a head is its elements i and i + HD / 2, turned by pos[axis[i]][t] * turns[i] turns
- * (1 turn = 2 pi; the product in 64 bits, its fraction in 32): y_i = x_i cos - x_(i + HD/2) sin, y_(i + HD/2) =
+ * (1 turn = 2 pi; the product's fraction in 64 bits, its sine and cosine in 32): y_i = x_i cos - x_(i + HD/2) sin, y_(i + HD/2) =
  * x_(i + HD/2) cos + x_i sin. With q_norm / k_norm, x is first x * rsqrt(mean(x^2) + eps) * (1 + w), as everywhere in
  * this library. 32-bit arithmetic, one rounding at the end.
  * slots == NULL: k goes to k_out and v is not looked at. Otherwise token t's k and v go to row slots[t] % page_rows of page
@@ -374,13 +376,13 @@ typedef struct {
   int32_t NQ, NK;          /* heads of q, and of k and v; 0 .. 1024, not both 0 */
   int32_t HD;              /* 64 or 128 */
   int32_t axes;            /* 1 .. 16 */
-  int32_t dtype;           /* mkx_dtype of q, k, v, the norm weights, outputs and pages */
+  int32_t dtype;           /* mkx_dtype of q, k, v, the norm weights, outputs and pages, and flags */
   float eps;
   const void* q, *k, *v;   /* [T, N, HD] */
   int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;
   void* q_out, *k_out;     /* [T, N, HD] */
   int64_t qo_stride_t, qo_stride_h, ko_stride_t, ko_stride_h;
-  const int32_t* pos;      /* [axes, T] */
+  const int32_t* pos;      /* [axes, T]; of int64_t with MKX_ROPE_POS64 */
   int64_t pos_stride;      /* elements between axes, >= T */
   const int32_t* axis;     /* [HD / 2] axis of each pair; outside [0, axes): axis 0 */
   const double* turns;     /* [HD / 2] turns per position */

@@ -164,8 +164,10 @@ __global__ __launch_bounds__(ROPE_BLOCK) void rope_kernel(mkx_rope_args a, int s
     const int t = i / HALF, p = i % HALF;
     int ax = a.axis[p];
     if (ax < 0 || ax >= a.axes) ax = 0;
-    const double turns = (double)a.pos[ax * a.pos_stride + t0 + t] * a.turns[p];
-    sincospif(2.0f * (float)(turns - rint(turns)), &s_sin[t][p], &s_cos[t][p]);
+    const int64_t at = ax * a.pos_stride + t0 + t;
+    const double x = a.dtype & MKX_ROPE_POS64 ? (double)((const int64_t*)a.pos)[at] : (double)a.pos[at], w = a.turns[p];
+    const double part = fma(x, w, -rint(x * w));  // the product unrounded: a far position keeps its fraction
+    sincospif(2.0f * (float)(part - rint(part)), &s_sin[t][p], &s_cos[t][p]);
   }
   __syncthreads();
   const int per = heads * UH;

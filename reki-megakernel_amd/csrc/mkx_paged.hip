@@ -21,20 +21,22 @@ int page_shift(int rows) {  // -1: not a page size
   return -1;
 }
 
+int type_of(const mkx_rope_args& a) { return a.dtype & ~MKX_ROPE_POS64; }
+
 // The n tokens (or as many as there are) from t0 on
 mkx_rope_args rope_from(mkx_rope_args a, int64_t t0, int64_t n) {
   auto skip = [&](const void* p, int64_t stride) { return (void*)((uintptr_t)p + 2 * (uintptr_t)(t0 * stride)); };
   a.T = (int)(a.T - t0 < n ? a.T - t0 : n);
   a.q = skip(a.q, a.q_stride_t), a.k = skip(a.k, a.k_stride_t), a.v = skip(a.v, a.v_stride_t);
   a.q_out = skip(a.q_out, a.qo_stride_t), a.k_out = skip(a.k_out, a.ko_stride_t);
-  a.pos += t0;
+  a.pos += a.dtype & MKX_ROPE_POS64 ? 2 * t0 : t0;
   if (a.slots != nullptr) a.slots += t0;
   return a;
 }
 
 hipError_t launch_rope(const mkx_rope_args& a, int shift, int tok, hipStream_t st) {
   const dim3 grid((unsigned)((a.T + tok - 1) / tok)), block(ROPE_BLOCK);
-  if (a.dtype == MKX_BF16) {
+  if (type_of(a) == MKX_BF16) {
     if (a.HD == 128) hipLaunchKernelGGL((rope_kernel<BF16, 128>), grid, block, 0, st, a, shift, tok);
     else hipLaunchKernelGGL((rope_kernel<BF16, 64>), grid, block, 0, st, a, shift, tok);
   } else {
@@ -75,11 +77,12 @@ int mkx_rope_axes(const mkx_rope_args* a, void* stream) {
   const char* me = "mkx_rope_axes";
   if (!a) return set_error(MKX_EINVAL, me, "args is NULL");
   if (a->HD != 64 && a->HD != 128) return set_error(MKX_EUNSUPPORTED, me, "HD must be 64 or 128");
-  if (a->dtype != MKX_BF16 && a->dtype != MKX_FP16) return set_error(MKX_EUNSUPPORTED, me, "dtype must be MKX_BF16 or MKX_FP16");
+  if (type_of(*a) != MKX_BF16 && type_of(*a) != MKX_FP16) return set_error(MKX_EUNSUPPORTED, me, "dtype must be MKX_BF16 or MKX_FP16");
   if (a->T < 0 || a->NQ < 0 || a->NK < 0 || a->NQ > 1024 || a->NK > 1024 || a->NQ + a->NK == 0 || a->axes < 1 || a->axes > 16)
     return set_error(MKX_EINVAL, me, "need T >= 0, heads of 0 .. 1024 (not both 0), axes of 1 .. 16");
   if (a->T > INT32_MAX - 64) return set_error(MKX_EINVAL, me, "T too large");
   if (!a->pos || !a->axis || !a->turns) return set_error(MKX_EINVAL, me, "pos, axis and turns are required");
+  if (((uintptr_t)a->pos & (a->dtype & MKX_ROPE_POS64 ? 7u : 3u)) != 0) return set_error(MKX_EINVAL, me, "pos is not aligned to its numbers");
   if (a->pos_stride < a->T && a->axes > 1) return set_error(MKX_EINVAL, me, "pos_stride smaller than T");
   if (!(a->eps >= 0.f)) return set_error(MKX_EINVAL, me, "eps must not be negative");
   const bool store = a->slots != nullptr;

@@ -24,8 +24,8 @@ import math
 
 import torch
 
-from ._lib import (BF16, EINVAL, FP16, MAX_SLOTS, OK, MkxAttendArgs, MkxPageMapArgs, MkxRopeArgs, check, lib, packer,
-                   require_device)
+from ._lib import (BF16, EINVAL, FP16, MAX_SLOTS, OK, MkxAttendArgs, MkxPageMapArgs, MkxRopeArgs, ROPE_POS64, check, lib,
+                   packer, require_device)
 
 PAGE_ROWS = (16, 32, 64, 128, 256)
 _DTYPES = {torch.bfloat16: BF16, torch.float16: FP16}
@@ -281,12 +281,13 @@ class AxesRotary:
         if len(n) != 2 or n[0] != self.axes or n[1] != T or pt not in (torch.int32, torch.int64):
             raise ValueError(f"pos must be [{self.axes}, {T}] int32 or int64, got {tuple(n)} {pt}")
         pa, one = pos.stride()
-        if pt != torch.int32 or one != 1 or pa < T:
-            pos = pos.to(torch.int32).contiguous()
+        if one != 1 or pa < T:
+            pos = pos.contiguous()
             pa = T
+        kind = _DTYPES[dt] | (ROPE_POS64 if pt == torch.int64 else 0)
         if T:
             wq, wk = self._norms.get(dt, _NONE)
-            a = _rope_args(T, NQ, NK, hd, self.axes, _DTYPES[dt], self.eps, qp, kp, vp, qs, qh, ks, kh, vs, vh, qo, ko, os, oh, us, uh,
+            a = _rope_args(T, NQ, NK, hd, self.axes, kind, self.eps, qp, kp, vp, qs, qh, ks, kh, vs, vh, qo, ko, os, oh, us, uh,
                            pos.data_ptr(), pa, self._axis_ptr, self._turns_ptr, 0 if wq is None else wq.data_ptr(),
                            0 if wk is None else wk.data_ptr(), sl, pages_k, pages_v, ps, pr, ph, n_pages, rows)
             _launch(lib().mkx_rope_axes, ctypes.byref(a), dev, "mkx_rope_axes")
@@ -294,7 +295,7 @@ class AxesRotary:
 
     def __call__(self, q: torch.Tensor | None, k: torch.Tensor | None, pos: torch.Tensor, q_out: torch.Tensor | None = None,
                  k_out: torch.Tensor | None = None):
-        """(q, k) [T, heads, head_dim] normed and turned by pos [axes, T] ([T] for one axis); either may be None. ``q_out`` /
+        """(q, k) [T, heads, head_dim] normed and turned by pos [axes, T] ([T] for one axis; int32 or int64); either may be None. ``q_out`` /
         ``k_out``: where the results go (q and k themselves too)."""
         return self._call(q, k, None, pos, q_out, k_out, None, None, None)
 

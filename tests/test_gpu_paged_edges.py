@@ -1,13 +1,15 @@
 """The paged cache's operators in calls beside the ordinary ones: requests that were not granted, positions and weights of other
 types, sizes at the launch's limits, the attention's other kernel."""
+import math
 import random
+from fractions import Fraction
 
 import pytest
 import torch
 
 from mkx.paged import AxesRotary, PagedCache, page_attend
 
-from _paged_ref import attend_ref
+from _paged_ref import HALF, attend_ref
 from test_gpu_paged import BF, DEV, FP, Att, _near, i32
 
 pytestmark = pytest.mark.gpu
@@ -141,3 +143,45 @@ def test_attention_of_more_rows_than_a_launch_has_workgroups_for(lead):
     assert bool((out[lead + 3: lead + 9] == 4).all())
     del out
     torch.cuda.empty_cache()
+
+
+# ---- rotary: positions and weights as they are given ----------------------------------------------------------------------------
+
+def _far_turns(rope, pos, hd):
+    """(cos, sin) [T, 1, hd / 2] of positions of any size: the turns' fractions as whole numbers give them, in 64 bits after that."""
+    turns, axis = [Fraction(x) for x in rope._turns.tolist()], rope._axis.tolist()
+    frac = torch.tensor([[float(Fraction(int(pos[a, t])) * turns[i] % 1) for i, a in enumerate(axis)] for t in range(pos.shape[1])], dtype=torch.float64)
+    ang = 2 * math.pi * frac[:, None]
+    return torch.cos(ang), torch.sin(ang)
+
+
+@pytest.mark.parametrize("layout", ["plain", "strided", "one_axis"])
+@pytest.mark.parametrize("store", [False, True])
+def test_rope_positions_beyond_32_bits(layout, store):
+    """64-bit positions turn by their own angle, whatever their upper half holds."""
+    HD, T, axes = 64, 40, 1 if layout == "one_axis" else 3
+    g = torch.Generator().manual_seed(5)
+    rope = AxesRotary(HD, [0] * 32 if axes == 1 else AxesRotary.sections((10, 11, 11)), device=DEV)
+    pos = torch.randint(-(1 << 44), 1 << 44, (axes, T), generator=g)
+    pos[:, :8] = torch.tensor([0, -1, (1 << 31) - 1, 1 << 31, -(1 << 31), (1 << 32) + 3, 1 << 52, -(1 << 40) - 7])
+    posd = pos.to(DEV)
+    if layout == "strided":
+        posd = torch.stack([posd, posd + 1], -1).flatten(1)[:, ::2]
+        assert posd.stride(1) == 2
+    elif layout == "one_axis":
+        posd = posd[0]
+    x = torch.randn(T, 3, HD, generator=g).to(BF)
+    xd = x.to(DEV)
+    if store:
+        kp, vp = (torch.zeros(3, 16, 3, HD, dtype=BF, device=DEV) for _ in range(2))
+        rope.store(None, xd, xd, posd, kp, vp, torch.arange(T, device=DEV))
+        got = kp.view(-1, 3, HD)[:T]
+    else:
+        got = rope(xd, None, posd)[0]
+    c, s = _far_turns(rope, pos, HD)
+    lo, hi = x[..., :32].double(), x[..., 32:].double()
+    want = torch.cat([lo * c - hi * s, hi * c + lo * s], -1)
+    # as in rope_ref: the fraction of a turn, its sine and cosine and the products in 32 bits; the product of position and turns
+    # is exact up to 2^-53 of its own rounding's size
+    mix = lo.abs() + hi.abs()
+    _near(got, want, HALF[BF] * want.abs() * (1 + 2.0 ** -8) + 2.0 ** -20 * torch.cat([mix, mix], -1))

@@ -5,7 +5,7 @@ import pytest
 
 from mkx import _lib
 
-from test_paged import P16, SIZES, _attend_args
+from test_paged import P16, SIZES, _attend_args, _rope_args
 
 
 @pytest.mark.parametrize("over,status", SIZES + [(dict(q=None), _lib.EINVAL), (dict(ws=P16 + 16), _lib.EINVAL), (dict(out=P16), _lib.EINVAL)])
@@ -15,3 +15,12 @@ def test_attention_of_granted_requests_refuses(over, status):
     assert "mkx_page_attend_granted:" in L.mkx_last_error().decode()
     assert L.mkx_page_attend_granted(None, P16, None) == _lib.EINVAL
     assert L.mkx_page_attend_granted(ctypes.byref(_attend_args(T=0)), P16, None) == _lib.OK
+
+
+@pytest.mark.parametrize("over,status", [
+    (dict(dtype=2 | _lib.ROPE_POS64), _lib.EUNSUPPORTED), (dict(dtype=_lib.BF16 | 2 * _lib.ROPE_POS64 | 4 * _lib.ROPE_POS64), _lib.EUNSUPPORTED),
+    (dict(dtype=_lib.FP16 | _lib.ROPE_POS64, pos=P16 + 4), _lib.EINVAL), (dict(pos=P16 + 2), _lib.EINVAL), (dict(dtype=_lib.BF16 | _lib.ROPE_POS64, pos_stride=3), _lib.EINVAL)])
+def test_rope_of_64_bit_positions_refuses(over, status):
+    L = _lib.lib()
+    assert L.mkx_rope_axes(ctypes.byref(_rope_args(**over)), None) == status, L.mkx_last_error()
+    assert L.mkx_rope_axes(ctypes.byref(_rope_args(T=0, dtype=_lib.FP16 | _lib.ROPE_POS64)), None) == _lib.OK
