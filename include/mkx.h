@@ -320,8 +320,10 @@ int mkx_modulation_input_ws(const mkx_modin_args* args, float* ws, void* stream)
  * [n_pages, page_rows, NK, HD]; request slot b owns the pages of row b of the block table, table[b][j] holding its tokens
  * j * page_rows and on. Calls are asynchronous on `stream`, allocate nothing, and can be captured. 16-bit types: */
 typedef enum { MKX_BF16 = 0, MKX_FP16 = 1 } mkx_dtype;
-/* Added to mkx_rope_args.dtype: pos is int64_t (8-byte aligned; beyond 2^53 a position is taken as the nearest double). */
+/* Added to mkx_rope_args.dtype: pos is int64_t (8-byte aligned; beyond 2^53 a position is taken as the nearest double); q_norm and
+ * k_norm are float, for models whose weights have more bits than their tokens or do not sit around 0. */
 #define MKX_ROPE_POS64 256
+#define MKX_ROPE_NORM32 512
 #define MKX_MAX_SLOTS 2048
 
 /* Block tables and slots of one step, from the requests' lengths. Request slot b has len_in[b] tokens and appends
@@ -386,8 +388,8 @@ typedef struct {
   int64_t pos_stride;      /* elements between axes, >= T */
   const int32_t* axis;     /* [HD / 2] axis of each pair; outside [0, axes): axis 0 */
   const double* turns;     /* [HD / 2] turns per position */
-  const void* q_norm;      /* [HD] or NULL */
-  const void* k_norm;      /* [HD] or NULL */
+  const void* q_norm;      /* [HD] or NULL; of float with MKX_ROPE_NORM32 */
+  const void* k_norm;      /* [HD] or NULL; as q_norm */
   const int64_t* slots;    /* [T] or NULL */
   void* k_pages, *v_pages; /* [n_pages, page_rows, NK, HD] with the strides below, both arrays */
   int64_t page_stride, row_stride, head_stride;

@@ -209,8 +209,14 @@ __global__ __launch_bounds__(ROPE_BLOCK) void rope_kernel(mkx_rope_args a, int s
         if (UH == 8) ss += dpp<0x141>(ss);  // row_half_mirror: the other quad of the half-row
         const float inv = rsqrtf(ss * (1.0f / HD) + a.eps);
         float wl[8], wh[8];
-        unpack8e<E>(ld16((const uint16_t*)w + c), wl);
-        unpack8e<E>(ld16((const uint16_t*)w + HALF + c), wh);
+        if (a.dtype & MKX_ROPE_NORM32) {
+          const float* wf = (const float*)w + c;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) wl[i] = wf[i], wh[i] = wf[HALF + i];
+        } else {
+          unpack8e<E>(ld16((const uint16_t*)w + c), wl);
+          unpack8e<E>(ld16((const uint16_t*)w + HALF + c), wh);
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           lo[i] = lo[i] * inv * (1.0f + wl[i]);

@@ -21,7 +21,7 @@ int page_shift(int rows) {  // -1: not a page size
   return -1;
 }
 
-int type_of(const mkx_rope_args& a) { return a.dtype & ~MKX_ROPE_POS64; }
+int type_of(const mkx_rope_args& a) { return a.dtype & ~(MKX_ROPE_POS64 | MKX_ROPE_NORM32); }
 
 // The n tokens (or as many as there are) from t0 on
 mkx_rope_args rope_from(mkx_rope_args a, int64_t t0, int64_t n) {

@@ -23,7 +23,7 @@ EXPORTS = ("mkx_create", "mkx_run", "mkx_check", "mkx_barriers", "mkx_set_profil
            "mkx_page_attend_granted")
 PROBE_BARRIER, PROBE_HANDOFF = 0, 1
 BF16, FP16 = 0, 1
-ROPE_POS64 = 256
+ROPE_POS64, ROPE_NORM32 = 256, 512
 MAX_SLOTS = 2048
 
 _vp = ctypes.c_void_p

@@ -24,13 +24,12 @@ import math
 
 import torch
 
-from ._lib import (BF16, EINVAL, FP16, MAX_SLOTS, OK, MkxAttendArgs, MkxPageMapArgs, MkxRopeArgs, ROPE_POS64, check, lib,
-                   packer, require_device)
+from ._lib import (BF16, EINVAL, FP16, MAX_SLOTS, OK, MkxAttendArgs, MkxPageMapArgs, MkxRopeArgs, ROPE_NORM32, ROPE_POS64, check,
+                   lib, packer, require_device)
 
 PAGE_ROWS = (16, 32, 64, 128, 256)
 _DTYPES = {torch.bfloat16: BF16, torch.float16: FP16}
 _rope_args, _attend_args = packer(MkxRopeArgs), packer(MkxAttendArgs)
-_NONE = (None, None)
 
 
 # the current stream's pointer without a Stream object around it, which takes 1.8 us a call: as long as some launches run;
@@ -205,8 +204,9 @@ class PagePool:
 class AxesRotary:
     """Rotary positions of several axes. ``axis_of_pair``: the axis that turns each of the head_dim / 2 pairs (pair i =
     elements i and i + head_dim / 2; ``sections`` makes the usual lists); the pair's frequency is theta^(-2 i / head_dim),
-    or ``freqs[i]`` radians per position. ``q_norm`` / ``k_norm``: [head_dim] weights of per-head RMS norms ahead of the turn
-    (used as 1 + w), or None."""
+    or ``freqs[i]`` radians per position. ``q_norm`` / ``k_norm``: [head_dim] weights of per-head RMS norms ahead of the turn, or
+    None. They are copied, and used as 1 + w: a model of plain weights passes w - 1, made in 32 bits. Weights of the
+    tokens' type are read as they are, others in 32 bits."""
 
     def __init__(self, head_dim: int, axis_of_pair, theta: float = 10000.0, freqs=None, q_norm: torch.Tensor | None = None,
                  k_norm: torch.Tensor | None = None, eps: float = 1e-6, device="cuda"):
@@ -227,7 +227,12 @@ class AxesRotary:
             if w is not None and tuple(w.shape) != (head_dim,):
                 raise ValueError(f"{name} must be [{head_dim}]")
         require_device(dev, q_norm=q_norm, k_norm=k_norm)
-        self._norms = {dt: tuple(None if w is None else w.detach().to(dt, copy=True).contiguous() for w in (q_norm, k_norm)) for dt in _DTYPES}
+        self._norms = {}  # of each tokens' type: its flag, the weights
+        given = [w.dtype for w in (q_norm, k_norm) if w is not None]
+        for dt in _DTYPES:
+            as_is = all(t == dt for t in given)
+            self._norms[dt] = (0 if as_is else ROPE_NORM32, *(None if w is None else w.detach().to(dt if as_is else torch.float32, copy=True).contiguous()
+                                                              for w in (q_norm, k_norm)))
 
     @staticmethod
     def sections(sizes, interleaved: bool = False) -> list:
@@ -284,9 +289,9 @@ class AxesRotary:
         if one != 1 or pa < T:
             pos = pos.contiguous()
             pa = T
-        kind = _DTYPES[dt] | (ROPE_POS64 if pt == torch.int64 else 0)
         if T:
-            wq, wk = self._norms.get(dt, _NONE)
+            kind, wq, wk = self._norms[dt]
+            kind |= _DTYPES[dt] | (ROPE_POS64 if pt == torch.int64 else 0)
             a = _rope_args(T, NQ, NK, hd, self.axes, kind, self.eps, qp, kp, vp, qs, qh, ks, kh, vs, vh, qo, ko, os, oh, us, uh,
                            pos.data_ptr(), pa, self._axis_ptr, self._turns_ptr, 0 if wq is None else wq.data_ptr(),
                            0 if wk is None else wk.data_ptr(), sl, pages_k, pages_v, ps, pr, ph, n_pages, rows)

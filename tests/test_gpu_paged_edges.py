@@ -9,7 +9,7 @@ import torch
 
 from mkx.paged import AxesRotary, PagedCache, page_attend
 
-from _paged_ref import HALF, attend_ref
+from _paged_ref import HALF, attend_ref, rope_ref
 from test_gpu_paged import BF, DEV, FP, Att, _near, i32
 
 pytestmark = pytest.mark.gpu
@@ -185,3 +185,30 @@ def test_rope_positions_beyond_32_bits(layout, store):
     # is exact up to 2^-53 of its own rounding's size
     mix = lo.abs() + hi.abs()
     _near(got, want, HALF[BF] * want.abs() * (1 + 2.0 ** -8) + 2.0 ** -20 * torch.cat([mix, mix], -1))
+
+
+@pytest.mark.parametrize("HD,dt,wt", [(64, BF, torch.float32), (128, FP, torch.float32), (128, BF, torch.float64), (64, BF, FP), (128, FP, BF)])
+def test_rope_norm_weights_of_other_types(HD, dt, wt):
+    """Weights of more bits than the tokens, or of the other 16-bit type, are not rounded to the tokens' type: plain weights near
+    0.1, passed as w - 1, keep their place."""
+    g = torch.Generator().manual_seed(9)
+    T = 37
+    plain = 0.1 + 0.01 * torch.randn(HD, generator=g, dtype=torch.float64)
+    wq, wk = ((plain - 1).to(wt), (torch.randn(HD, generator=g) * 1e-3).to(wt))
+    rope = AxesRotary(HD, [0] * (HD // 2), q_norm=wq.to(DEV), k_norm=wk.to(DEV), eps=1e-5, device=DEV)
+    x = torch.randn(T, 5, HD, generator=g).to(dt)
+    pos = torch.arange(T, dtype=torch.int32)[None]
+    freqs = 10000.0 ** (-torch.arange(0, HD, 2, dtype=torch.float64) / HD)
+    q, k = rope(x[:, :3].to(DEV), x[:, 3:].to(DEV), pos.to(DEV))
+    for got, part, w in ((q, x[:, :3], wq), (k, x[:, 3:], wk)):
+        want, tol = rope_ref(part, pos, [0] * (HD // 2), freqs, w, 1e-5)
+        # 1 + w in 32 bits: 2^-24 of the sum's 1, which is 2^-20 of a weight of 0.07 and more
+        _near(got, want, tol)
+    # one of them of the tokens' type, the other not
+    rope = AxesRotary(HD, [0] * (HD // 2), q_norm=wq.to(DEV), k_norm=wk.to(dt).to(DEV), eps=1e-5, device=DEV)
+    q2, k2 = rope(x[:, :3].to(DEV), x[:, 3:].to(DEV), pos.to(DEV))
+    want, tol = rope_ref(x[:, 3:], pos, [0] * (HD // 2), freqs, wk.to(dt), 1e-5)
+    _near(k2, want, tol)
+    assert torch.equal(q2, q)
+    both = AxesRotary(HD, [0] * (HD // 2), q_norm=wk.to(dt).to(DEV), k_norm=wk.to(dt).to(DEV), eps=1e-5, device=DEV)
+    assert torch.equal(both(None, x[:, 3:].to(DEV), pos.to(DEV))[1], k2)
