@@ -14,8 +14,8 @@ step's tokens over the cache, causal or not, with a sliding window and first tok
         q = cache.store(l, rope, q, k, v, pos, m)      # rotary and store, one launch
         o = cache.attend(l, q, m, max_q=..., window=..., sinks=...)
 
-All calls run on the current stream of their tensors' GPU and can be captured in a HIP graph. Nothing here runs without
-libmkx.so.
+All calls run on the current stream of their tensors' GPU and can be captured in a HIP graph. None has a backward pass: inputs
+that require grad are refused, unless gradients are off. Nothing here runs without libmkx.so.
 """
 from __future__ import annotations
 
@@ -48,6 +48,13 @@ def _launch(fn, args, device: torch.device, where: str) -> None:
             rc = fn(args, _stream(index))
     if rc != OK:
         check(rc, where)
+
+
+def _no_grad(**tensors) -> None:
+    """The operators serve: none has a backward pass, and a result without a graph would pass for a constant."""
+    for name, t in tensors.items():
+        if t is not None and t.requires_grad:
+            raise ValueError(f"{name} requires grad, and this has no backward pass: call it under torch.no_grad(), or detach {name}")
 
 
 def _gpu(device) -> torch.device:
@@ -256,6 +263,8 @@ class AxesRotary:
         for t in (q, k, v, pos, q_out, k_out, k_pages, v_pages, slots):
             if t is not None and t.get_device() != index:  # -1 on the host
                 require_device(dev, q=q, k=k, v=v, pos=pos, q_out=q_out, k_out=k_out, k_pages=k_pages, v_pages=v_pages, slots=slots)
+        if torch.is_grad_enabled():
+            _no_grad(q=q, k=k, v=v, q_out=q_out, k_out=k_out, k_pages=k_pages, v_pages=v_pages)
         NQ = NK = qs = qh = ks = kh = vs = vh = os = oh = us = uh = qp = kp = vp = qo = ko = pages_k = pages_v = ps = pr = ph = n_pages = rows = sl = 0
         dt = T = None
         if q is not None:
@@ -332,6 +341,8 @@ def page_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
     for t in (k_pages, v_pages, table, cu, kv_len, out, granted):
         if t is not None and t.get_device() != index:
             require_device(q.device, k_pages=k_pages, v_pages=v_pages, table=table, cu=cu, kv_len=kv_len, out=out, granted=granted)
+    if torch.is_grad_enabled():
+        _no_grad(q=q, k_pages=k_pages, v_pages=v_pages, out=out)
     dt = q.dtype
     q, shape, qs, qh, qp = _heads(q, "q", hd)
     T, NQ, _ = shape

@@ -212,3 +212,31 @@ def test_rope_norm_weights_of_other_types(HD, dt, wt):
     assert torch.equal(q2, q)
     both = AxesRotary(HD, [0] * (HD // 2), q_norm=wk.to(dt).to(DEV), k_norm=wk.to(dt).to(DEV), eps=1e-5, device=DEV)
     assert torch.equal(both(None, x[:, 3:].to(DEV), pos.to(DEV))[1], k2)
+
+
+# ---- gradients ------------------------------------------------------------------------------------------------------------------
+
+def test_inputs_that_require_grad_are_refused():
+    """No operator here has a backward pass: an input that asks for one is refused aloud, and served under no_grad."""
+    t = Att([3], [20], 4, 2, 64, 16, BF)
+    rope = AxesRotary(64, [0] * 32, q_norm=torch.nn.Parameter(torch.zeros(64, device=DEV, dtype=BF)), device=DEV)
+    x, pos = torch.randn(3, 2, 64, device=DEV).to(BF), torch.arange(3, dtype=torch.int32, device=DEV)
+    slots = torch.arange(3, device=DEV)
+    leaf = lambda y: y.clone().requires_grad_()  # noqa: E731
+    calls = {"q": lambda: rope(leaf(x), x, pos), "k": lambda: rope(x, leaf(x), pos),
+             "v": lambda: rope.store(x, x, leaf(x), pos, t.kp, t.vp, slots), "q_out": lambda: rope(x, None, pos, q_out=leaf(x)),
+             "k_out": lambda: rope(None, x, pos, k_out=leaf(x)), "k_pages": lambda: rope.store(x, x, x, pos, leaf(t.kp), t.vp, slots),
+             "v_pages": lambda: rope.store(x, x, x, pos, t.kp, leaf(t.vp), slots)}
+    attend = lambda **kw: page_attend(*[kw.get(n, y) for n, y in (("q", t.qd), ("k_pages", t.kp), ("v_pages", t.vp))],  # noqa: E731
+                                      t.table, t.cu, t.kv, out=kw.get("out"))
+    more = {"q": lambda: attend(q=leaf(t.qd)), "k_pages": lambda: attend(k_pages=leaf(t.kp)), "v_pages": lambda: attend(v_pages=leaf(t.vp)),
+            "out": lambda: attend(out=leaf(t.qd))}
+    for name, call in [*calls.items(), *more.items()]:
+        with torch.enable_grad(), pytest.raises(ValueError, match=f"^{name} requires grad"):
+            call()
+        with torch.no_grad():
+            call()
+    with torch.enable_grad():  # a weight may, it was copied
+        assert not rope(x, x, pos)[0].requires_grad and not attend().requires_grad
+    with torch.inference_mode():
+        rope(leaf(x), x, pos), attend()
