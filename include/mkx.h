@@ -370,8 +370,8 @@ int mkx_page_map(const mkx_page_map_args* args, void* stream);
  * this library. 32-bit arithmetic, one rounding at the end.
  * slots == NULL: k goes to k_out and v is not looked at. Otherwise token t's k and v go to row slots[t] % page_rows of page
  * slots[t] / page_rows; a slot outside [0, n_pages * page_rows) stores nothing, and of two tokens with one slot either may
- * be left there, in parts. NQ or NK may be 0 (its pointers are
- * then ignored). q_out may be q and k_out may be k with the same strides; outputs overlap inputs in no other way. Strides
+ * be left there, in parts. NQ or NK may be 0 (its pointers are then ignored). q_out may be q and k_out may be k with the
+ * same strides; outputs overlap inputs and each other in no other way (views of one buffer that do are refused). Strides
  * are in elements; every pointer to 16-bit numbers is 16-byte aligned and their strides are multiples of 8. */
 typedef struct {
   int32_t T;               /* tokens, >= 0 */

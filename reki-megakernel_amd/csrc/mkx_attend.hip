@@ -5,6 +5,7 @@
 #include "mkx_attend.h"
 
 #include "mkx_error.h"
+#include "mkx_overlap.h"
 
 using namespace mkx;
 
@@ -97,6 +98,8 @@ int attend(const char* me, const mkx_attend_args* a, const int32_t* granted, voi
   if (((uintptr_t)a->ws & 255u) != 0 || a->ws_bytes < 256)
     return set_error(MKX_EINVAL, me, "ws must be 256-byte aligned and hold mkx_page_attend_workspace() bytes");
   if (a->T == 0) return MKX_OK;
+  if (share_elements({a->q, a->NQ, a->q_stride_t, a->q_stride_h}, {a->out, a->NQ, a->o_stride_t, a->o_stride_h}, a->T, a->HD))
+    return set_error(MKX_EINVAL, me, "out shares elements with q");
   int cus;
   const int no_cus = cus_here(me, &cus);
   if (no_cus != MKX_OK) return no_cus;

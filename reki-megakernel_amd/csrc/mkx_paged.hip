@@ -2,6 +2,7 @@
 #include "mkx_paged.h"
 
 #include "mkx_error.h"
+#include "mkx_overlap.h"
 
 using namespace mkx;
 
@@ -121,6 +122,14 @@ int mkx_rope_axes(const mkx_rope_args* a, void* stream) {
     }
   }
   if (a->T == 0) return MKX_OK;
+  const View q = {a->q, a->NQ, a->q_stride_t, a->q_stride_h}, k = {a->k, a->NK, a->k_stride_t, a->k_stride_h},
+             v = {a->v, a->NK, a->v_stride_t, a->v_stride_h}, qo = {a->q_out, a->NQ, a->qo_stride_t, a->qo_stride_h},
+             ko = {a->k_out, a->NK, a->ko_stride_t, a->ko_stride_h};
+  auto shared = [&](const View& x, const View& y) { return share_elements(x, y, a->T, a->HD); };
+  if (a->NQ > 0 && ((q.p != qo.p && shared(q, qo)) || (a->NK > 0 && (shared(k, qo) || (store && shared(v, qo))))))
+    return set_error(MKX_EINVAL, me, "q_out shares elements with k or v, or with q without being q");
+  if (a->NK > 0 && !store && ((k.p != ko.p && shared(k, ko)) || (a->NQ > 0 && (shared(q, ko) || shared(qo, ko)))))
+    return set_error(MKX_EINVAL, me, "k_out shares elements with q or q_out, or with k without being k");
   // as many tokens a workgroup as leave its threads a unit each (30000 tokens of 4 + 1 heads of 128: 17.9 us, with one token
   // each 27.6, with half as many 21.6; 1100 tokens of 16 + 2 heads: one token each 4.5 us, four 5.4)
   const int units = (a->NQ + (store ? 2 : 1) * a->NK) * (a->HD / 16), fit = ROPE_BLOCK / units;

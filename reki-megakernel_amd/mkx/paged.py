@@ -310,7 +310,7 @@ class AxesRotary:
     def __call__(self, q: torch.Tensor | None, k: torch.Tensor | None, pos: torch.Tensor, q_out: torch.Tensor | None = None,
                  k_out: torch.Tensor | None = None):
         """(q, k) [T, heads, head_dim] normed and turned by pos [axes, T] ([T] for one axis; int32 or int64); either may be None. ``q_out`` /
-        ``k_out``: where the results go (q and k themselves too)."""
+        ``k_out``: where the results go: q and k themselves, or memory that no input or other result has."""
         return self._call(q, k, None, pos, q_out, k_out, None, None, None)
 
     def store(self, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, k_pages: torch.Tensor,
@@ -328,7 +328,7 @@ def page_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
     """Attention of new tokens over the paged cache: q [T, NQ, head_dim], slot b's tokens at cu[b] .. cu[b + 1] - 1 and at the
     end of its kv_len[b] cached tokens (their own k and v stored before). causal with ``window`` > 0: a token sees the last
     ``window`` tokens up to itself and the request's first ``sinks``. ``max_q``: a bound of the chunks' lengths that the
-    caller knows (1 for answered tokens), which shapes the launch only. ``out``: where the result goes; rows behind the
+    caller knows (1 for answered tokens), which shapes the launch only. ``out``: where the result goes, not an input's memory; rows behind the
     last slot's tokens are left as they are there (and unset without it). ``granted`` (``PageMap.granted``): slots with 0 were
     refused their tokens, which are not in the cache; their rows are zeros."""
     shape = q.shape

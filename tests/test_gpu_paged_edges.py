@@ -7,6 +7,7 @@ from fractions import Fraction
 import pytest
 import torch
 
+from mkx import _lib
 from mkx.paged import AxesRotary, PagedCache, page_attend
 
 from _paged_ref import HALF, attend_ref, rope_ref
@@ -240,3 +241,28 @@ def test_inputs_that_require_grad_are_refused():
         assert not rope(x, x, pos)[0].requires_grad and not attend().requires_grad
     with torch.inference_mode():
         rope(leaf(x), x, pos), attend()
+
+
+# ---- outputs in their inputs' buffers ------------------------------------------------------------------------------------------
+
+
+def test_outputs_beside_inputs_in_one_buffer():
+    """Results that go between the heads of their inputs, or before and behind them, are no overlap."""
+    g = torch.Generator().manual_seed(8)
+    rope = AxesRotary(64, [0] * 32, device=DEV)
+    x = torch.randn(40, 12, 64, generator=g).to(BF).to(DEV)
+    pos = torch.arange(40, dtype=torch.int32, device=DEV)
+    q, k = rope(x[:, :3], x[:, 6:9], pos)
+    y = x.clone()
+    rope(y[:, :3], y[:, 6:9], pos, q_out=y[:, 3:6], k_out=y[:, 9:])
+    assert torch.equal(y[:, 3:6], q) and torch.equal(y[:, 9:], k) and torch.equal(y[:, :3], x[:, :3]) and torch.equal(y[:, 6:9], x[:, 6:9])
+    for out in (y[:, 1:4], y[:, 5:8]):
+        with pytest.raises(_lib.MkxError, match="shares elements"):
+            rope(y[:, :3], y[:, 6:9], pos, q_out=out, k_out=y[:, 9:])
+    t = Att([40], [40], 4, 2, 64, 16, BF)
+    both = torch.zeros(41, 8, 64, dtype=BF, device=DEV)
+    both[:40, :4] = t.qd
+    assert torch.equal(page_attend(both[:40, :4], t.kp, t.vp, t.table, t.cu, t.kv, out=both[:40, 4:]), t.run())
+    for out in (both[1:, :4], both[:40, 2:6]):
+        with pytest.raises(_lib.MkxError, match="shares elements"):
+            page_attend(both[:40, :4], t.kp, t.vp, t.table, t.cu, t.kv, out=out)
