@@ -127,7 +127,8 @@ class PagePool:
     """Which pages of a paged cache belong to which request slot. ``map(add, done)`` makes the tables of a step in which slot b
     appends add[b] tokens, or has ended (done[b] != 0: its pages return); ``commit()`` makes the last map the pool's
     state; ``append`` does both. A request is granted its tokens as a whole or not at all (``PageMap.granted``): its pages
-    have to fit its table row and the free pages, in the order of the slots. Lengths never visit the host."""
+    have to fit its table row, and the pages that it and the slots before it asked for have to be free; a slot that is
+    refused pages holds up the later ones that need some until it is passed with add = 0. Lengths never visit the host."""
 
     def __init__(self, slots: int, n_pages: int, page_rows: int, table_cols: int, max_tokens: int, device="cuda"):
         if not 1 <= slots <= MAX_SLOTS:

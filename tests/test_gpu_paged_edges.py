@@ -8,9 +8,9 @@ import pytest
 import torch
 
 from mkx import _lib
-from mkx.paged import AxesRotary, PagedCache, page_attend
+from mkx.paged import AxesRotary, PagedCache, PagePool, page_attend
 
-from _paged_ref import HALF, attend_ref, rope_ref
+from _paged_ref import HALF, attend_ref, map_ref, rope_ref
 from test_gpu_paged import BF, DEV, FP, Att, _near, i32
 
 pytestmark = pytest.mark.gpu
@@ -266,3 +266,26 @@ def test_outputs_beside_inputs_in_one_buffer():
     for out in (both[1:, :4], both[:40, 2:6]):
         with pytest.raises(_lib.MkxError, match="shares elements"):
             page_attend(both[:40, :4], t.kp, t.vp, t.table, t.cu, t.kv, out=out)
+
+
+# ---- who waits for whom -----------------------------------------------------------------------------------------------------------
+
+def test_map_refused_needs_hold_up_later_slots():
+    """A prompt that lacks pages counts against the slots behind it: those that need a page are refused with it, those that need none
+    are not; with add = 0 for the prompt they pass. Tokens count against max_tokens whether granted or not, pages that no table
+    row holds against nobody."""
+    P, cols, N, T = 16, 4, 6, 90
+    pool = PagePool(4, N, P, cols, T, DEV)
+    length, table, queue, head, free = [0] * 4, [[-1] * cols for _ in range(4)], list(range(N)), 0, N
+    for add, granted in (([0, 16, 20, 0], [1, 1, 1, 1]),      # 3 pages taken, 3 free
+                         ([50, 1, 1, 1], [0, 0, 1, 0]),       # 4 are too many; then 1 more each, though 3 are free; slot 2 needs none
+                         ([0, 1, 1, 1], [1, 1, 1, 1]),        # 1 free
+                         ([41, 1, 19, 0], [0, 1, 0, 1]),      # 3 pages, then 1 more; slot 1 needs none
+                         ([75, 0, 1, 16], [0, 1, 1, 0]),      # more than a row holds; slot 3's tokens end behind T
+                         ([65, 0, 0, 16], [0, 1, 1, 1])):     # the same, and slot 3 gets the last page
+        want = map_ref(add, None, length, head, free, table, queue, P, T)
+        assert want["granted"] == granted, add
+        m = pool.append(i32(add))
+        for name, w in want.items():
+            assert getattr(m, name).tolist() == w, (add, name)
+        length, table, queue, (head, free) = want["kv_len"], want["table"], want["queue"], want["ends"]
