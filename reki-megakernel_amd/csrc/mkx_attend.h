@@ -84,22 +84,26 @@ __device__ __forceinline__ args_ptr fresh(args_ptr p) {
   return p;
 }
 
+typedef const __attribute__((address_space(4))) AttendLaunch* launch_ptr;
+__device__ __forceinline__ launch_ptr launch_at(args_ptr p) {
+  return (launch_ptr)((const __attribute__((address_space(4))) char*)p + sizeof(mkx_attend_args));
+}
 __device__ __forceinline__ AttendLaunch launch_args(args_ptr p) {
-  const auto* l = (const __attribute__((address_space(4))) AttendLaunch*)((const __attribute__((address_space(4))) char*)p + sizeof(mkx_attend_args));
-  return AttendLaunch{l->shift, l->G, l->bm, l->parts, l->tiles, l->stamp, l->granted};
+  const launch_ptr l = launch_at(p);
+  return AttendLaunch{l->shift, l->G, l->bm, l->parts, l->tiles, l->stamp, nullptr};  // granted: read where the requests are, and no longer
 }
 static_assert(sizeof(mkx_attend_args) % 8 == 0, "AttendLaunch follows at its own alignment");
 
 struct Request {
   int q0, nq, n;  // first token, tokens, cached keys
 };
-template <class A>
-__device__ __forceinline__ Request request(A& a, const AttendLaunch& L, int b) {
-  const const_i32 cu = (const_i32)(uintptr_t)a.cu, kv = (const_i32)(uintptr_t)a.kv_len, granted = (const_i32)(uintptr_t)L.granted;
+__device__ __forceinline__ Request request(args_ptr pa, int shift, int b) {
+  const auto& a = *pa;
+  const const_i32 cu = (const_i32)(uintptr_t)a.cu, kv = (const_i32)(uintptr_t)a.kv_len, granted = (const_i32)(uintptr_t)launch_at(fresh(pa))->granted;
   Request r;
   r.q0 = min(max(cu[b], 0), a.T);
   r.nq = max(min(cu[b + 1], a.T) - r.q0, 0);
-  r.n = (int)min((int64_t)max(kv[b], 0), (int64_t)a.cols << L.shift);
+  r.n = (int)min((int64_t)max(kv[b], 0), (int64_t)a.cols << shift);
   if (granted != nullptr && granted[b] == 0) r.n = 0;  // its tokens are not in the cache
   return r;
 }
@@ -782,7 +786,7 @@ __global__ __launch_bounds__(ATT_BLOCK, 2) void attend_tiles_kernel(mkx_attend_a
     const int m = (b + e) >> 1;
     if (slot(m) <= tile) b = m; else e = m;
   }
-  const Request r = request(a, L, b);
+  const Request r = request(pa, L.shift, b);
   const int row0 = (tile - slot(b)) * L.bm;
   if (row0 < 0 || row0 >= r.nq * L.G) return;
   const Item it = make_item(a, L, r, b, h, row0);
@@ -952,7 +956,7 @@ __global__ __launch_bounds__(ATT_BLOCK, 2) void attend_kernel(mkx_attend_args, A
     const int b = tid & 63;
     Request r = {0, 0, 0};
     if (b < B) {
-      r = request(*pa, L, b);
+      r = request(pa, L.shift, b);
       keep(b, r);
     }
     const int nt = (r.nq * L.G + L.bm - 1) / L.bm;
@@ -993,7 +997,7 @@ __global__ __launch_bounds__(ATT_BLOCK, 2) void attend_kernel(mkx_attend_args, A
       const int b = tid * per_b + i;
       req[i] = Request{0, 0, 0};
       if (i < per_b && b < B) {
-        req[i] = request(*pa, L, b);
+        req[i] = request(pa, L.shift, b);
         keep(b, req[i]);
         const int tiles = (req[i].nq * L.G + L.bm - 1) / L.bm;
         nt = min(nt + tiles, ATT_TILES);
