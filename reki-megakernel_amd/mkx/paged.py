@@ -50,10 +50,12 @@ def _launch(fn, args, device: torch.device, where: str) -> None:
         check(rc, where)
 
 
-def _no_grad(**tensors) -> None:
-    """The operators serve: none has a backward pass, and a result without a graph would pass for a constant."""
+def _require(device: torch.device, **tensors) -> None:
+    """Tensors of the operators' GPU, and without gradients to make: none has a backward pass, and a result without a graph would
+    pass for a constant."""
+    require_device(device, **tensors)
     for name, t in tensors.items():
-        if t is not None and t.requires_grad:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} requires grad, and this has no backward pass: call it under torch.no_grad(), or detach {name}")
 
 
@@ -262,10 +264,8 @@ class AxesRotary:
             raise ValueError("nothing to turn: q or k is needed")
         index = dev.index
         for t in (q, k, v, pos, q_out, k_out, k_pages, v_pages, slots):
-            if t is not None and t.get_device() != index:  # -1 on the host
-                require_device(dev, q=q, k=k, v=v, pos=pos, q_out=q_out, k_out=k_out, k_pages=k_pages, v_pages=v_pages, slots=slots)
-        if torch.is_grad_enabled():
-            _no_grad(q=q, k=k, v=v, q_out=q_out, k_out=k_out, k_pages=k_pages, v_pages=v_pages)
+            if t is not None and (t.get_device() != index or t.requires_grad):  # -1 on the host
+                _require(dev, q=q, k=k, v=v, pos=pos, q_out=q_out, k_out=k_out, k_pages=k_pages, v_pages=v_pages, slots=slots)
         NQ = NK = qs = qh = ks = kh = vs = vh = os = oh = us = uh = qp = kp = vp = qo = ko = pages_k = pages_v = ps = pr = ph = n_pages = rows = sl = 0
         dt = T = None
         if q is not None:
@@ -339,11 +339,9 @@ def page_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
     index = q.get_device()
     if index < 0:
         raise ValueError(f"q is on {q.device}: the paged cache sits on a GPU")
-    for t in (k_pages, v_pages, table, cu, kv_len, out, granted):
-        if t is not None and t.get_device() != index:
-            require_device(q.device, k_pages=k_pages, v_pages=v_pages, table=table, cu=cu, kv_len=kv_len, out=out, granted=granted)
-    if torch.is_grad_enabled():
-        _no_grad(q=q, k_pages=k_pages, v_pages=v_pages, out=out)
+    for t in (q, k_pages, v_pages, table, cu, kv_len, out, granted):
+        if t is not None and (t.get_device() != index or t.requires_grad):
+            _require(q.device, q=q, k_pages=k_pages, v_pages=v_pages, table=table, cu=cu, kv_len=kv_len, out=out, granted=granted)
     dt = q.dtype
     q, shape, qs, qh, qp = _heads(q, "q", hd)
     T, NQ, _ = shape
