@@ -409,8 +409,11 @@ int mkx_rope_axes(const mkx_rope_args* args, void* stream);
  * whatever they hold, infinities and NaN too; a table entry outside [0, n_pages) in their place
  * reads as keys and values of zeros. Lengths outside their ranges are clamped. The products take 16-bit operands and
  * accumulate in 32 bits, softmax statistics are 32-bit, the probabilities are rounded to the type of v.
- * max_q: an upper bound of every slot's chunk that the caller knows, or T; it shapes the launch (and with it the order of
- * sums), and a bound that is too low costs time only. row_stride is at most 2^27.
+ * max_q: an upper bound of every slot's chunk that the caller knows, or T. It and T shape the launch (and with it the order of
+ * sums), and a bound that is too low costs time only: tiles have bm = 64, 128 or 256 rows, for up to 64, 128 or more rows
+ * max_q NQ / NK of a slot; with T NQ / NK / bm + B above 2048, or with tiles of 256 rows for two workgroups a CU and more, a tile has a
+ * workgroup of its own and the keys of a few rows are not split. row_stride is at most 2^27. A value that is infinite, and
+ * that every row of a tile sees, may give NaN where its probability rounds to 0.
  * ws: mkx_page_attend_workspace() bytes, 256-byte aligned, of this call alone until it has run. The same call on the
  * same inputs gives the same bits. */
 typedef struct {

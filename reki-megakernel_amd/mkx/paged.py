@@ -120,7 +120,8 @@ class PageMap:
     int64 cache row of each token (-1: none), ``pos`` [max_tokens] the token's index in its request, ``granted`` [B],
     ``kv_len`` [B] lengths after the step, ``ends`` [2] head and number of the free pages after it, ``table`` and ``queue``
     (the pool's). A map's tensors are written again by the pool's second map after a commit, and by its next map without
-    one."""
+    one. Replays of captured maps write the same sets without the pool object's knowing: its own view is right after as many
+    replays of the one set as of the other."""
 
     __slots__ = ("cu", "slots", "pos", "granted", "kv_len", "ends", "table", "queue")
 
@@ -329,7 +330,8 @@ def page_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
     """Attention of new tokens over the paged cache: q [T, NQ, head_dim], slot b's tokens at cu[b] .. cu[b + 1] - 1 and at the
     end of its kv_len[b] cached tokens (their own k and v stored before). causal with ``window`` > 0: a token sees the last
     ``window`` tokens up to itself and the request's first ``sinks``. ``max_q``: a bound of the chunks' lengths that the
-    caller knows (1 for answered tokens), which shapes the launch only. ``out``: where the result goes, not an input's memory; rows behind the
+    caller knows (1 for answered tokens); it and q's rows shape the launch only, but many more rows than the step can have
+    keep the keys of a few tokens from being split. ``out``: where the result goes, not an input's memory; rows behind the
     last slot's tokens are left as they are there (and unset without it). ``granted`` (``PageMap.granted``): slots with 0 were
     refused their tokens, which are not in the cache; their rows are zeros."""
     shape = q.shape
