@@ -150,8 +150,8 @@ __global__ __launch_bounds__(MAP_BLOCK) void page_map_kernel(mkx_page_map_args a
 // Bound by memory: a token's heads are read once and written once. A workgroup takes `tok` tokens; their angles are made
 // once (a thread a pair: the turns in 64 bits, their fraction through sincospi in 32) and shared by all heads through
 // LDS, and a thread moves 8 pairs of a head at a time (16 bytes of either half), so that a head is HD / 16 neighbouring
-// lanes and its norm a sum over them. 30011 tokens of 32 + 8 heads of 128, stored: 132 us, 5.6 TB/s (a 2 GiB copy on this
-// card 4.9); 16 tokens of 16 + 2 heads 3.1 us in a graph.
+// lanes and its norm a sum over them. 30011 tokens of 32 + 8 heads of 128, stored: 133 us, 5.5 TB/s (a 2 GiB copy on this
+// card 4.9); 16 tokens of 16 + 2 heads 3.3 us in a graph.
 constexpr int ROPE_BLOCK = 256, ROPE_TOK = 16;  // threads; tokens of a workgroup at most
 
 template <class E, int HD>
