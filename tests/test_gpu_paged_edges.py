@@ -10,7 +10,7 @@ import torch
 from mkx import _lib
 from mkx.paged import AxesRotary, PagedCache, PagePool, page_attend
 
-from _paged_ref import HALF, attend_ref, map_ref, rope_ref
+from _paged_ref import HALF, attend_ref, map_ref, rope_ref, sees
 from test_gpu_paged import BF, DEV, FP, Att, _near, i32
 
 pytestmark = pytest.mark.gpu
@@ -289,3 +289,84 @@ def test_map_refused_needs_hold_up_later_slots():
         for name, w in want.items():
             assert getattr(m, name).tolist() == w, (add, name)
         length, table, queue, (head, free) = want["kv_len"], want["table"], want["queue"], want["ends"]
+
+
+def test_pool_after_replays_of_both_graphs():
+    """The pool's own view, a load and eager appends between replays: right after as many replays of the one graph as of the other."""
+    P, cols, N, T, B = 16, 5, 12, 50, 3
+    pool = PagePool(B, N, P, cols, T, DEV)
+    add, done = i32([0] * B), i32([0] * B)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        pool.append(add, done), pool.append(add, done)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, maps = [], []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            maps.append(pool.append(add, done))
+        graphs.append(gr)
+    state = [0] * B, [[-1] * cols for _ in range(B)], list(range(N)), 0, N
+    saved = None
+    todo = [([9, 20, 0], "g"), ([9, 1, 16], "g"), ([1, 1, 1], "e"), ([0, 30, 1], "e"), ([2, 0, 1], "g"), ([-1, 3, 1], "g"), ([5, 5, 5], "e"), ([1, 0, 0], "e")]
+    for i, (a, how) in enumerate(todo):
+        ended = [0, 0, int(i == 3)]
+        add.copy_(i32(a)), done.copy_(i32(ended))
+        want = map_ref(a, ended, *state[:1], state[3], state[4], state[1], state[2], P, T)
+        if how == "g":
+            graphs[i % 2].replay()
+            m = maps[i % 2]
+        else:
+            m = pool.append(add, done)
+        for name, w in want.items():
+            assert getattr(m, name).tolist() == w, (i, name)
+        state = want["kv_len"], want["table"], want["queue"], *want["ends"]
+        if i % 2:
+            assert pool.kv_len.tolist() == state[0] and pool.ends.tolist() == list(state[3:])
+            got = pool.state_dict()
+            if i == 3:
+                saved = got, state
+    pool.load_state_dict(saved[0])
+    state = saved[1]
+    for i, a in enumerate(([4, 4, 4], [1, 1, 1])):
+        add.copy_(i32(a)), done.zero_()
+        want = map_ref(a, None, state[0], state[3], state[4], state[1], state[2], P, T)
+        graphs[i].replay()
+        for name, w in want.items():
+            assert getattr(maps[i], name).tolist() == w, (i, name)
+        state = want["kv_len"], want["table"], want["queue"], *want["ends"]
+
+
+# ---- keys that are not numbers ------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("HD,dt,G,NK,max_q", [(128, BF, 8, 2, 40), (64, FP, 1, 3, 40), (128, FP, 4, 40, None), (64, BF, 8, 1, 5)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_attention_keys_that_only_some_rows_see(HD, dt, G, NK, max_q, bad):
+    """NaN and infinite keys of the chunk itself and at the window's edge, under NaN queries of other tokens: the rows that see
+    them are no numbers, the others what they are without."""
+    nq, n, W, S = [40, 3, 1, 200], [300, 260, 77, 390], 37, 5
+    t = Att(nq, n, NK * G, NK, HD, 16, dt, seed=G)
+    spoilt = {(0, 290): 0, (0, 255): NK - 1, (1, 258): 0, (1, 2): 0, (3, 380): 0, (3, 388): NK - 1, (3, 120): 0}
+    for (b, j), h in spoilt.items():
+        t.k[b][j, h] = bad
+        t.kp[t.table_l[b][j // 16], j % 16, h] = bad
+    dead = {(0, 3), (3, 77), (3, 199)}  # these queries themselves
+    for b, i in dead:
+        t.q[t.cu_l[b] + i] = float("nan")
+        t.qd[t.cu_l[b] + i] = float("nan")
+    for window, sinks in ((0, 0), (W, S)):
+        out = t.run(window=window, sinks=sinks, max_q=max_q).double().cpu()
+        for b, q in enumerate(nq):
+            live = t.q[t.cu_l[b]: t.cu_l[b + 1]].nan_to_num(0.0)
+            o, tol = attend_ref(live, t.k[b].nan_to_num(0.0, 0.0, 0.0), t.v[b], True, window, sinks, HD ** -0.5)
+            got = out[t.cu_l[b]: t.cu_l[b + 1]]
+            no = torch.zeros(q, NK, dtype=torch.bool)
+            for i in range(q):
+                for (c, j), h in spoilt.items():
+                    no[i, h] |= c == b and sees(n[b] - q + i, j, n[b], True, window, sinks)
+                no[i] |= (b, i) in dead
+            no = no.repeat_interleave(G, 1)
+            if bad != bad:
+                assert bool(torch.isnan(got[no]).all()), b
+            _near(got[~no], o[~no], tol[~no], (b, window))
